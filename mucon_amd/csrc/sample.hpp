@@ -74,7 +74,8 @@ struct Drawing {
         const float v = a.uniform[r];
         u = !(v > 0.f) ? 0.0 : v >= 1.f ? 0.99999994039535522 : (double)v;
     }
-    __device__ __forceinline__ bool greedy() const { return !(it > 0.0) || k == 1; }
+    // (a top_p of nothing keeps the first of the order: no running sum is asked where it reaches a number that it has from the start)
+    __device__ __forceinline__ bool greedy() const { return !(it > 0.0) || k == 1 || top_p <= 0.f; }
 };
 template <int TY>
 __device__ __forceinline__ bool no_distribution(uint32_t top) { return top >= key_inf<TY>() || top <= key_ninf<TY>(); }
