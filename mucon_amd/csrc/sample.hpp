@@ -45,7 +45,7 @@ struct SampleShared {
             uint32_t count[BINS];
         };
     };
-    u64 found[4];
+    u64 found[5];
 };
 struct CountShared {
     uint32_t times[PAGES * PAGE / 2];            // two 16-bit counters a word
@@ -512,7 +512,8 @@ __device__ __forceinline__ Crossing cross_bins(RowIn<TY, NT, 0> &in, const Weigh
     // its elements: few of the row, told apart by fp32 values a little wider than the bin before the bin itself is computed
     const float far_x = (float)(wg.top - (double)(bin + 1) / (BINS_PER_OCTAVE * wg.octaves)), near_x = (float)(wg.top - (double)bin / (BINS_PER_OCTAVE * wg.octaves));
     const float slack = 1e-6f * (fabsf(far_x) + fabsf(near_x) + fabsf((float)wg.top));
-    const float low = bin == BINS - 1 ? -INFINITY : far_x - slack, high = near_x + slack;
+    const bool told = slack < INFINITY;      // (at temperatures near the largest fp32 a border lies behind every number: the bin itself tells all of them apart)
+    const float low = bin == BINS - 1 || !told ? -INFINITY : far_x - slack, high = told ? near_x + slack : INFINITY;
     if (tid == 0) sh.sel.n = 0;
     __syncthreads();
     in.each([&](const Vec &v, int i) {
@@ -541,13 +542,13 @@ __device__ __forceinline__ Crossing cross_bins(RowIn<TY, NT, 0> &in, const Weigh
             run += wg.units(value_of_key<TY>(key_of(sh.sel.list[i])));
             const bool at = COUNT ? past(cbase + i + 1) && (i == 0 || !past(cbase + i)) : past(run) && (i == 0 || !past(had));
             if (at) {      // (one thread: the sums do not fall)
-                sh.found[2] = run;
                 sh.found[3] = i;
+                sh.found[4] = run;
             }
         }
         __syncthreads();
         const u64 c0 = sh.sel.list[min(sh.found[3], (u64)max(n - 1, 0))];
-        return Crossing{sh.found[2], index_of(c0), value_of_key<TY>(key_of(c0))};
+        return Crossing{sh.found[4], index_of(c0), value_of_key<TY>(key_of(c0))};
     }
     // too many alike: the crossing value bit by bit of its key within the bin, then the place among its equals
     uint32_t t = 0;
