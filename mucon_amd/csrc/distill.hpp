@@ -4,8 +4,11 @@
 //   p_k = softmax over the listed (no teacher log-sum-exp given), or exp(a_k - lse) with the rest p_r = max(0, 1 - sum p_k) on the tokens that are not listed, together;
 //   L   = T^2 [ sum_k p_k (log p_k - log q_k) + p_r (log p_r - log q_r) ],   q_r = sum of q over the tokens that are not listed;
 //   dL / ds_j = T [ q_j (P - [j not listed] p_r / q_r) - sum_{k: i_k = j} p_k ],   P = sum p_k + p_r.
-// q_r is summed over the tokens whose bit is not set in an LDS bitmap, never taken as 1 - sum q_k, which cancels.  Where no mass is left outside the list there is no rest
-// term.  Sums over the vocabulary and the logarithms of the listed entries, which are subtracted from each other, are held in 64 bits; the exponentials of a row are fp32.
+// With a rest, the unlisted tokens (those whose bit is not set in an LDS bitmap) are summed against their own maximum m_o and the listed ones against theirs: q_r is never
+// taken as 1 - sum q_k, which cancels, and is as good where it is e^-1000 of the row, as where a student is certain of what its teacher doubts.  Their part of the gradient,
+//   T exp((s_j - m_o) / T) [P exp((m_o - m) / T) / Z - p_r / Zo],   Z the row's sum against its maximum m, Zo = sum_unlisted exp((s - m_o) / T) >= 1,
+// has no large factor.  Only where no unlisted token is above -inf is there no rest term.  Sums over the vocabulary and the logarithms of the listed entries, which are
+// subtracted from each other, are held in 64 bits; the exponentials of a row are fp32.
 #pragma once
 #include "row_common.hpp"
 #include "top_rows.hpp"
@@ -13,8 +16,8 @@
 namespace rows {
 
 struct DistillRow {   // what the gradient of a row needs
-    float m;          // the row's maximum
-    float in, out;    // dL / ds_j = T (in or out) exp((s_j - m) / T) - T p: for the listed tokens, for the others
+    float m, mo;      // the row's maximum, that of the unlisted tokens (no rest: the row's)
+    float in, out;    // dL / ds_j = T in exp((s_j - m) / T) - T p for the listed tokens, T out exp((s_j - mo) / T) for the others
     float used;       // 0: a row without weight
     double lp0;       // log p_k = a_k - lp0
 };
@@ -49,23 +52,36 @@ struct ListSums {
     double S, A, B;    // sum e_k, sum e_k (a_k - shift), sum e_k s_k / T
 };
 
-// The end of a row, by one wave: from the sums over its tokens (Z; Zo: those not listed, of exp((s - m) / T)) and over the list.  The three logarithms side by side in
-// three lanes: one after the other they are a third of a short row's time.
-__device__ __forceinline__ DistillRow finish_row(const ListSums &l, double Z, double Zo, double shift, float m, double temperature, bool rest, double *loss) {
+// What the tokens of a row add up to.  Without a rest every token counts as unlisted.
+struct TokenSums {
+    double Zo, Zl;     // of exp((s - mo) / T) over the unlisted tokens, of exp((s - ml) / T) over the listed ones
+    float mo, ml;      // their maxima, -inf where there is none
+};
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+// The end of a row, by one wave.  The two exponentials and then the three logarithms side by side in a lane each: one after the other they are a third of a short row's
+// time.
+__device__ __forceinline__ DistillRow finish_row(const ListSums &l, const TokenSums &z, double shift, double temperature, bool rest, double *loss) {
     const int lane = threadIdx.x & 63;
+    const float m = base_of(fmaxf(z.mo, z.ml));
+    const double below = exp(((double)(lane == 0 ? z.mo : z.ml) - (double)m) / temperature);
+    const double wo = __shfl(below, 0), wl = __shfl(below, 1);
+    const double Z = z.Zo * wo + (rest ? z.Zl * wl : 0.0);
     double pr = 1.0 - l.S;
-    pr = pr < 0.0 || Zo == 0.0 ? 0.0 : pr;      // (NaN stays)
-    const double logs = log(lane == 0 ? Z : lane == 1 ? Zo : rest ? pr : l.S);
+    pr = pr < 0.0 || z.Zo == 0.0 ? 0.0 : pr;      // (NaN stays)
+    const double logs = log(lane == 0 ? Z : lane == 1 ? z.Zo : rest ? pr : l.S);
     const double logZ = __shfl(logs, 0), log_out = __shfl(logs, 1), log_last = __shfl(logs, 2);
     const double B = l.B - l.S * ((double)m / temperature + logZ);      // sum e_k log q_k
     DistillRow st;
     st.m = m;
+    st.mo = rest ? base_of(z.mo) : m;
     st.used = 1.f;
     if (rest) {
-        *loss = l.A - B + (pr > 0.0 ? pr * (log_last - (log_out - logZ)) : pr);
+        const double log_qr = log_out + ((double)st.mo - (double)m) / temperature - logZ;
+        *loss = l.A - B + (pr > 0.0 ? pr * (log_last - log_qr) : pr);
         const double P = l.S + pr;
         st.in = (float)(P / Z);
-        st.out = (float)(P / Z - (pr > 0.0 ? pr / Zo : pr));
+        st.out = (float)(P * wo / Z - (pr > 0.0 ? pr / z.Zo : pr));
         st.lp0 = shift;
     } else {
         *loss = l.S == 0.0 ? 0.0 : (l.A - B) / l.S - log_last;
@@ -109,7 +125,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a, long 
         if (MODE && mine) store_one<TY>(out, lane, 0.f);
         if (MODE != 2 && lane == 0) {
             a.losses[r] = 0.f;
-            if (MODE == 0) a.stat[r] = DistillRow{0.f, 0.f, 0.f, 0.f, 0.0};
+            if (MODE == 0) a.stat[r] = DistillRow{0.f, 0.f, 0.f, 0.f, 0.f, 0.0};
         }
         return;
     }
@@ -123,16 +139,19 @@ __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a, long 
     if (MODE == 2) {
         st = a.stat[r];
     } else {
-        const float M = wave_reduce<MaxF>(x);
-        const float base = M == -INFINITY ? 0.f : M;
-        const float e = mine ? __builtin_amdgcn_exp2f((x - base) * c) : 0.f;
-        const double Z = wave_reduce<Sum>((double)e);
-        double Zo = 0.0, shift;
+        bool in = false;
+        double shift;
+        TokenSums z{0.0, 0.0, 0.f, -INFINITY};
         if (rest) {
-            bool in = false;
             for (int k = 0; k < a.k; ++k) in |= __shfl(index, k) == lane;
-            Zo = wave_reduce<Sum>(in ? 0.0 : (double)e);
+            z.ml = wave_reduce<MaxF>(in ? x : -INFINITY);
             shift = (double)a.lse[r];
+        }
+        z.mo = wave_reduce<MaxF>(in ? -INFINITY : x);
+        const float e = mine ? __builtin_amdgcn_exp2f((x - base_of(in ? z.ml : z.mo)) * c) : 0.f;
+        z.Zo = wave_reduce<Sum>(in ? 0.0 : (double)e);
+        if (rest) {
+            z.Zl = wave_reduce<Sum>(in ? (double)e : 0.0);
         } else {
             const float amax = wave_reduce<MaxF>(t);
             shift = amax == -INFINITY ? 0.0 : (double)amax / a.temperature;
@@ -147,7 +166,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a, long 
         l.A = wave_reduce<Sum>(l.A);
         l.B = wave_reduce<Sum>(l.B);
         double loss;
-        st = finish_row(l, Z, Zo, shift, base, a.temperature, rest, &loss);
+        st = finish_row(l, z, shift, a.temperature, rest, &loss);
         if (lane == 0) {
             a.losses[r] = (float)(loss * a.temperature * a.temperature * (double)weight);
             if (MODE == 0) a.stat[r] = st;
@@ -164,7 +183,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(DistillArgs a, long 
         in |= here;
         take += here ? pk : 0.f;
     }
-    const float e = __builtin_amdgcn_exp2f((x - st.m) * c);
+    const float e = __builtin_amdgcn_exp2f((x - (in ? st.m : st.mo)) * c);
     if (mine) store_one<TY>(out, lane, (float)(g * (double)(in ? st.in : st.out)) * e - take);
 }
 
@@ -175,15 +194,17 @@ struct RowList {      // the list in LDS
     uint32_t *bits;   // of the tokens that are listed
     double shift;
     ListSums own;     // this thread's entries
+    double Zl;        // ... and their tokens, each once, of exp((s - ml) / T) (with a rest)
+    float ml;         // the largest student logit of a listed token (with a rest)
 };
 struct ListShared {
     int again;        // whether a token is listed twice
-    uint32_t top;     // key of the largest listed logit
+    uint32_t top;     // key of the largest listed logit (no rest), of the largest student logit of a listed token (with one)
 };
 __host__ __device__ __forceinline__ int list_words(int vocab, int k) { return 2 * k + ((vocab + 31) >> 5); }
 
-// The list and its sums.  They need nothing of the row's maximum, so all of this runs while the row's loads are on their way.  The caller's next barrier stands before
-// the first use of e and bits.
+// The list and its sums.  They need nothing of the row's maximum, so all of this runs while the row's loads are on their way.  The bits stand when it returns; the caller's
+// next barrier stands before the first use of e.
 template <int TY, int NT>
 __device__ __forceinline__ RowList load_list(const DistillArgs &a, long long r, const char *row, uint32_t *lds, ListShared &sh) {
     RowList l;
@@ -204,26 +225,36 @@ __device__ __forceinline__ RowList load_list(const DistillArgs &a, long long r, 
         l.index[k] = ok ? j : -1;
         l.e[k] = t;
         if (ok && (atomicOr(&l.bits[j >> 5], 1u << (j & 31)) >> (j & 31) & 1)) sh.again = 1;
-        if (ok) top = max(top, key_of_bits<F32>(__float_as_uint(t)));
+        if (ok) top = max(top, a.lse ? key_of_bits<TY>(load_bits<TY>(row, j)) : key_of_bits<F32>(__float_as_uint(t)));
     }
+    if (top) atomicMax(&sh.top, top);
+    __syncthreads();
+    l.ml = -INFINITY;
     if (a.lse) {
         l.shift = (double)a.lse[r];
+        if (sh.top) l.ml = value_of_key<TY>(sh.top);
     } else {
-        if (top) atomicMax(&sh.top, top);
-        __syncthreads();
         l.shift = sh.top <= key_ninf<F32>() ? 0.0 : (double)value_of_key<F32>(sh.top) / a.temperature;
     }
     l.own = ListSums{0.0, 0.0, 0.0};
+    l.Zl = 0.0;
     for (int k = threadIdx.x; k < a.k; k += NT) {
         const int j = l.index[k];
         double e = 0.0;
         if (j >= 0) {
             const double d = (double)l.e[k] / a.temperature - l.shift;
             e = exp(d);
+            const double x = (double)value_of_bits<TY>(load_bits<TY>(row, j));
             if (e != 0.0) {
                 l.own.S += e;
                 l.own.A += e * d;
-                l.own.B += e * ((double)value_of_bits<TY>(load_bits<TY>(row, j)) / a.temperature);
+                l.own.B += e * (x / a.temperature);
+            }
+            if (a.lse && x != -INFINITY) {
+                bool first = true;      // (the token's first entry, so that the sum's order does not change)
+                if (sh.again)
+                    for (int q = 0; q < k; ++q) first &= l.index[q] != j;
+                if (first) l.Zl += exp((x - (double)l.ml) / a.temperature);
             }
         }
         l.e[k] = (float)e;
@@ -269,24 +300,25 @@ __device__ __forceinline__ void block_sums(double (&v)[C], double (*scratch)[16]
     }
 }
 
-// A vector's exponentials of (x - base) c: their sum, and that of the unlisted ones (in: the listed ones' bits; few vectors have any)
+// A vector without the listed tokens (in: their bits; few vectors have any)
 template <int TY>
-__device__ __forceinline__ void add_vector(const Vec &v, uint32_t in, float base, float c, bool rest, double &s, double &so) {
+__device__ __forceinline__ void hide_listed(Vec &v, uint32_t in) {
     constexpr int N = El<TY>::N;
-    float w[N], sum = 0.f;
+    if (!(in & ((1u << N) - 1))) return;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        w[e] = __builtin_amdgcn_exp2f((value_of<TY>(v, e) - base) * c);
-        sum += w[e];
+        const uint32_t mask = TY == F32 ? ~0u : (e & 1) ? 0xffff0000u : 0xffffu;
+        uint32_t &d = v.d[TY == F32 ? e : e >> 1];
+        if ((in >> e) & 1) d = (d & ~mask) | (El<TY>::LOWEST & mask);
     }
-    s += (double)sum;
-    if (!rest) return;
-    if (in & ((1u << N) - 1)) {
-        sum = 0.f;
+}
+// A vector's exponentials of (x - base) c, added up
+template <int TY>
+__device__ __forceinline__ void add_vector(const Vec &v, float base, float c, double &s) {
+    float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum += (in >> e) & 1 ? 0.f : w[e];
-    }
-    so += (double)sum;
+    for (int e = 0; e < El<TY>::N; ++e) sum += __builtin_amdgcn_exp2f((value_of<TY>(v, e) - base) * c);
+    s += (double)sum;
 }
 // A vector of a gradient row in which nothing is listed
 template <int TY>
@@ -300,7 +332,7 @@ template <int TY, int NT>
 __device__ void empty_row(const DistillArgs &a, long long r, bool grad) {
     if (threadIdx.x == 0) {
         a.losses[r] = 0.f;
-        a.stat[r] = DistillRow{0.f, 0.f, 0.f, 0.f, 0.0};
+        a.stat[r] = DistillRow{0.f, 0.f, 0.f, 0.f, 0.f, 0.0};
     }
     if (!grad) return;
     float x[El<TY>::N];
@@ -310,11 +342,11 @@ __device__ void empty_row(const DistillArgs &a, long long r, bool grad) {
     for (int i = threadIdx.x; i * El<TY>::N < a.vocab; i += NT) store_vec<TY>(out, i, a.vocab, x);
 }
 
-// The first wave, with the row's sums: its loss, and its record -- for the gradient of a later call, or (GRAD) of this workgroup, with what turns e_k into the gradient's p_k
+// The first wave, with the row's sums (Zo, Zl and the list's): its loss, and its record -- for the gradient of a later call, or (GRAD) of this workgroup, with what turns e_k into the gradient's p_k
 template <bool GRAD>
-__device__ __forceinline__ void end_row(const DistillArgs &a, long long r, const double (&all)[5], double shift, float m, bool rest, float weight, double g, DistillRow *row, float *gp) {
+__device__ __forceinline__ void end_row(const DistillArgs &a, long long r, const double (&all)[5], float mo, float ml, double shift, bool rest, float weight, double g, DistillRow *row, float *gp) {
     double loss;
-    const DistillRow st = finish_row(ListSums{all[2], all[3], all[4]}, all[0], all[1], shift, m, a.temperature, rest, &loss);
+    const DistillRow st = finish_row(ListSums{all[2], all[3], all[4]}, TokenSums{all[0], all[1], mo, ml}, shift, a.temperature, rest, &loss);
     if (threadIdx.x) return;
     a.losses[r] = (float)(loss * a.temperature * a.temperature * (double)weight);
     if (GRAD) {
@@ -355,25 +387,27 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     const bool rest = a.lse != nullptr;
     float m = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < NV; ++q)
+    for (int q = 0; q < NV; ++q) {
+        const int i = q * NT + tid;
+        if (rest && i < nvec) hide_listed<TY>(v[q], list.bits[(i * N) >> 5] >> ((i * N) & 31));
 #pragma unroll
         for (int e = 0; e < N; ++e) m = fmaxf(m, value_of<TY>(v[q], e));
+    }
     m = wave_reduce<MaxF>(m);
     if ((tid & 63) == 0) sf[tid >> 6] = m;
     __syncthreads();
     for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, sf[w]);
-    const float base = m == -INFINITY ? 0.f : m;
-    double s = 0.0, so = 0.0;
+    const float base = base_of(m);
+    double s = 0.0;
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-        const int i = q * NT + tid;
         forget(v[q]);
-        add_vector<TY>(v[q], rest && i < nvec ? list.bits[(i * N) >> 5] >> ((i * N) & 31) : 0, base, c, rest, s, so);
+        add_vector<TY>(v[q], base, c, s);
     }
-    double all[5] = {s, so, list.own.S, list.own.A, list.own.B};
+    double all[5] = {s, list.Zl, list.own.S, list.own.A, list.own.B};
     block_sums<NT, 5>(all, sd);
     const double g = GRAD ? grad_factor(a, r) : 0.0;
-    if (tid < 64) end_row<GRAD>(a, r, all, list.shift, base, rest, weight, g, &shared_row, &shared_gp);
+    if (tid < 64) end_row<GRAD>(a, r, all, m, list.ml, list.shift, rest, weight, g, &shared_row, &shared_gp);
     if (!GRAD) return;
     __syncthreads();
     const DistillRow st = shared_row;
@@ -384,7 +418,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
         const int i = q * NT + tid;
         forget(v[q]);
         float x[N];
-        grad_vector<TY>(v[q], base, c, fout, x);
+        grad_vector<TY>(v[q], st.mo, c, fout, x);
         if (i < nvec) store_vec<TY>(out, i, a.vocab, x);
     }
     __syncthreads();
@@ -413,7 +447,7 @@ __global__ __launch_bounds__(NT) void distill_stream_kernel(DistillArgs a) {
     const float c = (float)(1.4426950408889634 / a.temperature);
     const bool rest = a.lse != nullptr;
     float m = -INFINITY;
-    double s = 0.0, so = 0.0;
+    double s = 0.0;
     for (int first = tid; first < nvec; first += NT * AHEAD) {
         Vec v[AHEAD];
         float top = -INFINITY;
@@ -426,33 +460,27 @@ __global__ __launch_bounds__(NT) void distill_stream_kernel(DistillArgs a) {
                 v[q] = Vec{{El<TY>::LOWEST, El<TY>::LOWEST, El<TY>::LOWEST, El<TY>::LOWEST}};
         }
 #pragma unroll
-        for (int q = 0; q < AHEAD; ++q)
-#pragma unroll
-            for (int e = 0; e < N; ++e) top = fmaxf(top, value_of<TY>(v[q], e));
-        if (top > m) {
-            const double f = (double)__builtin_amdgcn_exp2f((m - top) * c);
-            s *= f;
-            so *= f;
-            m = top;
-        }
-        const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
             const int i = first + q * NT;
-            add_vector<TY>(v[q], rest && i < nvec ? list.bits[(i * N) >> 5] >> ((i * N) & 31) : 0, base, c, rest, s, so);
+            if (rest && i < nvec) hide_listed<TY>(v[q], list.bits[(i * N) >> 5] >> ((i * N) & 31));
+#pragma unroll
+            for (int e = 0; e < N; ++e) top = fmaxf(top, value_of<TY>(v[q], e));
         }
+        if (top > m) {
+            s *= (double)__builtin_amdgcn_exp2f((m - top) * c);
+            m = top;
+        }
+        const float base = base_of(m);
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) add_vector<TY>(v[q], base, c, s);
     }
     const float M = block_reduce<NT, MaxF>(m, sf);
-    const float base = M == -INFINITY ? 0.f : M;
-    if (m != M && s != 0.0) {   // (s is NaN where the thread met one)
-        const double f = (double)__builtin_amdgcn_exp2f((m - base) * c);
-        s *= f;
-        so *= f;
-    }
-    double all[5] = {s, so, list.own.S, list.own.A, list.own.B};
+    const float base = base_of(M);
+    if (m != M && s != 0.0) s *= (double)__builtin_amdgcn_exp2f((m - base) * c);   // (s is NaN where the thread met one)
+    double all[5] = {s, list.Zl, list.own.S, list.own.A, list.own.B};
     block_sums<NT, 5>(all, sd);
     const double g = GRAD ? grad_factor(a, r) : 0.0;
-    if (tid < 64) end_row<GRAD>(a, r, all, list.shift, base, rest, weight, g, &shared_row, &shared_gp);
+    if (tid < 64) end_row<GRAD>(a, r, all, M, list.ml, list.shift, rest, weight, g, &shared_row, &shared_gp);
     if (!GRAD) return;
     __syncthreads();
     const DistillRow st = shared_row;
@@ -466,7 +494,7 @@ __global__ __launch_bounds__(NT) void distill_stream_kernel(DistillArgs a) {
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
             float x[N];
-            grad_vector<TY>(v[q], base, c, fout, x);
+            grad_vector<TY>(v[q], st.mo, c, fout, x);
             if (first + q * NT < nvec) store_vec<TY>(out, first + q * NT, a.vocab, x);
         }
     }
@@ -532,7 +560,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillArgs a, int chun
     const float fout = (float)(g * (double)st.out), fin = (float)(g * (double)st.in);
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-        grad_vector<TY>(v[q], st.m, c, fout, x);
+        grad_vector<TY>(v[q], st.mo, c, fout, x);
         if (from + q * NT < nvec) store_vec<TY>(out, from + q * NT, a.vocab, x);
     }
     __syncthreads();

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import rows as orow
-from test_gpu_rows import U, check_drawn, cuda, host, rows_of
+from test_gpu_rows import U, check_distill, check_drawn, cuda, host, rows_of
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -71,3 +71,97 @@ def test_draws_of_logits_at_the_end_of_fp32():
         for k, p in ((0, 1.0), (600, 1.0), (0, 0.9), (5000, 0.9)):
             token, logp = ops.sample_logits(*cuda(x, u), torch.full((3,), T).cuda(), k, p)
             check_drawn(token.cpu(), logp.cpu(), host(x), u, (np.float32(T).item(), k, np.float32(p).item(), 0.0))
+
+
+# ------------------------------------------------------------------------------------------------ distillation
+def far_case(V, dtype, T, seed, levels, rest_mass=0.5, rows=4):
+    """Unlisted student logits within half a unit of 0, listed ones at `levels` (exact in every type); the teacher leaves `rest_mass` to the unlisted tokens."""
+    g = torch.Generator().manual_seed(seed)
+    s = torch.randint(-8, 9, (rows, V), generator=g).float() / 16.0
+    K = len(levels)
+    index = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(rows)]).to(torch.int32)
+    s.scatter_(1, index.long(), torch.tensor(levels).expand(rows, K))
+    values = torch.randint(-4, 5, (rows, K), generator=g).float() * (T / 4.0)
+    lse = (torch.logsumexp(values.double() / T, 1) - math.log(1.0 - rest_mass)).float()
+    return s.to(dtype), values, index, lse
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [7, 48, 64, 65, 900, 9000, 40000, 131072])
+@pytest.mark.parametrize("T,levels", [(0.1, [6.0, 12.0]), (0.1, [9.0, 9.0, 9.0]), (1.0, [95.0, 88.0]), (0.5, [-60.0, -100.0, -60.0]), (0.05, [8.0, 16.0, 24.0])])
+def test_distill_students_far_from_their_teacher(V, dtype, T, levels):
+    """The unlisted tokens' mass is e^-60 to e^-480 of the row's, below the smallest fp32: the rest term and its gradient are those of the definition, and finite (in the
+    fourth case it is the listed tokens' mass that is small)."""
+    from mucon_amd import ops
+
+    s, values, index, lse = far_case(V, dtype, T, V, levels)
+    leaf = s.cuda().requires_grad_(True)
+    d = cuda(values, index, lse)
+    for reduction in ("none", "sum"):
+        loss = ops.distill_loss(leaf, *d, temperature=T, reduction=reduction)
+        grad, = torch.autograd.grad(loss.sum(), leaf)
+        assert bool(grad.isfinite().all()) and bool(loss.isfinite().all())
+        check_distill(loss.detach(), grad, s, values, index, lse, None, T, reduction)
+        loss, grad = ops.distill_loss_and_grad(s.cuda(), *d, temperature=T, reduction=reduction, grad_scale=2.0)
+        check_distill(loss, grad, s, values, index, lse, None, T, reduction, torch.full((4,), 2.0) if reduction == "none" else 2.0)
+
+
+@pytest.mark.parametrize("V", [48, 900, 40000, 131072])
+def test_distill_of_a_far_row_under_a_loss_scale(V):
+    """A scaled loss, as for 16-bit gradients: the gradient of the definition times the scale."""
+    from mucon_amd import ops
+
+    T, scale = 0.1, 65536.0
+    for levels in ([8.25, 8.5], [8.5, 8.75], [8.75, 8.75]):      # e^-82 .. e^-88: around the smallest fp32
+        s, values, index, lse = far_case(V, torch.float32, T, V, levels)
+        leaf = s.cuda().requires_grad_(True)
+        d = cuda(values, index, lse)
+        loss = ops.distill_loss(leaf, *d, temperature=T, reduction="sum")
+        grad, = torch.autograd.grad(loss, leaf, torch.tensor(scale).cuda())
+        check_distill(loss.detach(), grad, s, values, index, lse, None, T, "sum", scale)
+        _, grad = ops.distill_loss_and_grad(s.cuda(), *d, temperature=T, reduction="sum", grad_scale=scale)
+        check_distill(loss.detach(), grad, s, values, index, lse, None, T, "sum", scale)
+
+
+@pytest.mark.parametrize("V", [48, 900, 40000, 131072])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_far_rows_whose_unlisted_tokens_rise(V, dtype):
+    """Unlisted logits that grow along the row, and listed ones between and above them, some listed twice, one of them -inf: the running maximum moves with every step."""
+    from mucon_amd import ops
+
+    T = 0.25
+    s = (torch.arange(V) * 32 // V).float().repeat(3, 1)
+    index = torch.tensor([[V - 1, 0, 3, 0], [V // 2, V // 2 + 1, -1, V // 2], [1, 2, 3, V]], dtype=torch.int32)
+    s[0, 0], s[0, 3], s[0, V - 1] = 80.0, 40.0, -math.inf
+    s[1, V // 2] = 64.0
+    s[2, 1:4] = torch.tensor([-40.0, 16.0, 120.0])
+    s = s.to(dtype)
+    values = torch.tensor([[-math.inf, 1.0, 0.0, 0.5], [0.0, 0.25, 9.0, 0.0], [0.5, 0.0, 0.25, 0.0]])
+    lse = torch.tensor([5.5, 3.0, 4.0])
+    leaf = s.cuda().requires_grad_(True)
+    d = cuda(values, index, lse)
+    loss = ops.distill_loss(leaf, *d, temperature=T, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    check_distill(loss.detach(), grad, s, values, index, lse, None, T, "none")
+    loss, grad = ops.distill_loss_and_grad(s.cuda(), *d, temperature=T, reduction="none")
+    check_distill(loss, grad, s, values, index, lse, None, T, "none")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_with_a_rest_at_a_low_temperature_and_far_from_zero(dtype):
+    """Logits around 60 at temperature 1/20 with the teacher's log-sum-exp given: near 1,200, where its own step in fp32 is 2^-13, which enters 1 - sum p as it is given."""
+    from mucon_amd import ops
+
+    for V in (48, 900, 40000):
+        g = torch.Generator().manual_seed(6)
+        s = (60.0 + 0.25 * torch.randint(-6, 7, (5, V), generator=g)).to(dtype)        # (exact in every type)
+        t = (60.0 + 0.25 * torch.randint(-6, 7, (5, V), generator=g)).to(dtype)
+        values, index = t.float().topk(5, dim=1)
+        lse = (torch.logsumexp(t.double() / 0.05, 1)).float()
+        values, index = values.to(dtype), index.to(torch.int32)
+        leaf = s.cuda().requires_grad_(True)
+        loss = ops.distill_loss(leaf, *cuda(values, index, lse), temperature=0.05, reduction="sum")
+        grad, = torch.autograd.grad(loss, leaf)
+        check_distill(loss.detach(), grad, s, values, index, lse, None, 0.05, "sum")
+        loss, grad = ops.distill_loss_and_grad(s.cuda(), *cuda(values, index, lse), temperature=0.05, reduction="sum")
+        check_distill(loss, grad, s, values, index, lse, None, 0.05, "sum")
