@@ -887,13 +887,16 @@ def _row_operand(t: torch.Tensor, like: torch.Tensor, shape, dtype, what: str) -
 
 
 def _on_device_of(fn):
-    """The call on the device of its first argument, where that is not the current one."""
+    """The call on the device of its first argument (given by place or by name), where that is not the current one."""
+    first = fn.__code__.co_varnames[0]
+
     @functools.wraps(fn)
-    def call(x, *args, **kw):
-        if x.is_cuda and x.get_device() != torch._C._cuda_getDevice():
+    def call(*args, **kw):
+        x = args[0] if args else kw.get(first)
+        if x is not None and x.is_cuda and x.get_device() != torch._C._cuda_getDevice():
             with torch.cuda.device(x.device):
-                return fn(x, *args, **kw)
-        return fn(x, *args, **kw)
+                return fn(*args, **kw)
+        return fn(*args, **kw)
     return call
 
 

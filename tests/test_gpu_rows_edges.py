@@ -165,3 +165,16 @@ def test_distill_with_a_rest_at_a_low_temperature_and_far_from_zero(dtype):
         check_distill(loss.detach(), grad, s, values, index, lse, None, 0.05, "sum")
         loss, grad = ops.distill_loss_and_grad(s.cuda(), *cuda(values, index, lse), temperature=0.05, reduction="sum")
         check_distill(loss, grad, s, values, index, lse, None, 0.05, "sum")
+
+
+# ------------------------------------------------------------------------------------------------ calls
+def test_the_operators_called_by_name():
+    from mucon_amd import ops
+
+    s, values, index, lse = far_case(300, torch.bfloat16, 1.0, 1, [1.0, 2.0, 0.5])
+    s, values, index, lse, u = cuda(s, values, index, lse, torch.rand(4))
+    assert all(torch.equal(a, b) for a, b in zip(ops.top_logits(logits=s, k=5), ops.top_logits(s, 5)))
+    assert all(torch.equal(a, b) for a, b in zip(ops.sample_logits(uniform=u, logits=s), ops.sample_logits(s, u)))
+    listed = dict(teacher_values=values, teacher_index=index, teacher_lse=lse)
+    assert torch.equal(ops.distill_loss(student=s, **listed), ops.distill_loss(s, values, index, lse))
+    assert all(torch.equal(a, b) for a, b in zip(ops.distill_loss_and_grad(student=s, **listed), ops.distill_loss_and_grad(s, values, index, lse)))

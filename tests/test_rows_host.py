@@ -146,3 +146,16 @@ def test_more_rows_than_a_launch_holds():
     cfg = _cfg(rows=1 << 20, vocab=1 << 18, row_stride=1 << 18, type=1)       # 1 M rows in 32 pieces each
     need = lib.mucon_distill_workspace_bytes(ctypes.byref(cfg))
     assert lib.mucon_distill_bwd(ctypes.byref(cfg), 64, 64, 64, 0, 0, 64, 64, 64, need, None) == _lib.E_ARG
+
+
+def test_every_argument_may_be_given_by_name():
+    """On host tensors: refused for being there, not for a missing argument."""
+    from mucon_amd import _lib, ops
+
+    x, listed = torch.zeros(2, 8), dict(teacher_values=torch.zeros(2, 2), teacher_index=torch.zeros(2, 2, dtype=torch.int32))
+    for fn, kw in ((ops.top_logits, dict(logits=x, k=2)), (ops.sample_logits, dict(logits=x, uniform=torch.zeros(2))), (ops.distill_loss, dict(student=x, **listed)),
+                   (ops.distill_loss_and_grad, dict(student=x, **listed))):
+        with pytest.raises(_lib.MuconHipError, match="no CPU fallback"):
+            fn(**kw)
+        with pytest.raises(TypeError, match="logits|student"):
+            fn(**{name: v for name, v in kw.items() if v is not x})
