@@ -390,18 +390,27 @@ class MuCon(nn.Module):
     @torch.no_grad()
     def sample_transcript(self, batch: Batch, uniform: Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """A transcript drawn word by word instead of the arg-max of forward(): step s runs the decoder over the words drawn so far and draws the next with uniform[s]
-        (ops.sample_logits).  uniform float32 [S] on the device, S <= max_decoding_steps.  -> (words up to and with the end mark, their log-probabilities).  One host
-        round trip, at the end."""
+        (ops.sample_logits).  uniform float32 [S] on the device, S <= max_decoding_steps.  -> (words up to and with the end mark, their log-probabilities).  No dropout
+        in the decoder.  One host round trip, at the end: all S words are drawn.  The native decoder starts from the first word at each of them (S (S + 1) / 2 decoder
+        steps, 496 for 31 words); where its sizes do not fit, or native_decoder is False, the module's own steps carry the state on."""
         steps = int(uniform.shape[0])
         if not 1 <= steps <= self.max_decoding_steps:
             raise ValueError(f"sample_transcript: {steps} uniforms for at most {self.max_decoding_steps} steps")
         memory, h_n, c_n = self._sequence_encoder(self.temporal_modeling_forward(input=batch.feats))
         words = torch.empty(steps + 1, dtype=torch.int64, device=batch.feats.device)
         words[0] = batch.transcript_tf_input[0]
+        native = self._native_decoder_ok(memory)
+        if not native:
+            state = self._decoder_start(memory, h_n, c_n)
         drawn, logps = [], []
         for s in range(steps):
-            logp, _ = ops.decoder_forward(memory[0], h_n, c_n, words[:s + 1], self._decoder_param_list(), s + 1, True, False, self.EOS_token_id)
-            word, word_logp = ops.sample_logits(logp[s], uniform[s], temperature, top_k, top_p, min_p)
+            if native:
+                logp, _ = ops.decoder_forward(memory[0], h_n, c_n, words[:s + 1], self._decoder_param_list(), s + 1, True, False, self.EOS_token_id)
+                row = logp[s]
+            else:
+                logp, _, state = self._decoder_step(words[s:s + 1], state, dropout=False)
+                row = logp[0]
+            word, word_logp = ops.sample_logits(row, uniform[s], temperature, top_k, top_p, min_p)
             drawn.append(word)
             logps.append(word_logp)
             words[s + 1] = word.clamp(min=0)      # (-1, a row without a distribution, is no embedding)
@@ -419,23 +428,13 @@ class MuCon(nn.Module):
         steps = tf_transcript_target_length if (self.teacher_forcing or self.training) else self.max_decoding_steps
         if self._native_decoder_ok(enc_out):
             return self._native_decoder(enc_out[0], h_n, c_n, steps, transcript_tf_input)
-        dec_h = self.fs_encoder_hidden_out(h_n.view(1, -1)).unsqueeze(0)   # [1 x 1 x D'']
-        dec_c = self.fs_encoder_cn_out(c_n.view(1, -1)).unsqueeze(0)
-        memory = enc_out[0]                                               # [Tz x 2D']
-        memory_proj = memory @ self.fs_decoder_attention_W1               # [Tz x D'']
+        state = self._decoder_start(enc_out, h_n, c_n)
         lengths, transcripts = [], []
         dec_in = transcript_tf_input[0].unsqueeze(0)
         for step in range(steps):
             if self.teacher_forcing:
                 dec_in = transcript_tf_input[step].unsqueeze(0)
-            emb = self.fs_decoder_embedding_drop(F.relu(self.fs_decoder_embedding(dec_in)))      # [1 x Ds]
-            attn = self._calculate_attention(dec_h, memory_proj)                                  # [Tz]
-            context = (attn.unsqueeze(1) * memory).sum(dim=0, keepdim=True)                       # [1 x 2Ds]
-            mixed = F.relu(self.fs_decoder_attn_combine(torch.cat((emb, context), 1)).unsqueeze(0))  # [1 x 1 x Ds]
-            dec_out, (dec_h, dec_c) = self.fs_decoder_lstm(mixed, (dec_h, dec_c))
-            word_logits = self.fs_decoder_transcript(dec_out)                                     # [1 x 1 x M+1]
-            length = self.fs_decoder_length(F.relu(torch.cat((mixed, word_logits), 2))).squeeze()
-            word_logp = F.log_softmax(word_logits.squeeze(0), dim=1)                              # [1 x M+1]
+            word_logp, length, state = self._decoder_step(dec_in, state)
             transcripts.append(word_logp)
             lengths.append(length)
             word = word_logp.argmax(dim=1)
@@ -444,6 +443,27 @@ class MuCon(nn.Module):
             if not self.teacher_forcing:
                 dec_in = word
         return transcripts, lengths
+
+    def _decoder_start(self, enc_out: Tensor, h_n: Tensor, c_n: Tensor):
+        """The state in front of the module decoder's first step: (h, c, memory, the memory as the attention reads it)."""
+        dec_h = self.fs_encoder_hidden_out(h_n.view(1, -1)).unsqueeze(0)   # [1 x 1 x D'']
+        dec_c = self.fs_encoder_cn_out(c_n.view(1, -1)).unsqueeze(0)
+        memory = enc_out[0]                                               # [Tz x 2D']
+        return dec_h, dec_c, memory, memory @ self.fs_decoder_attention_W1   # [Tz x D'']
+
+    def _decoder_step(self, dec_in: Tensor, state, dropout: bool = True):
+        """One step of the module decoder from the word dec_in [1]: (log-probabilities [1 x M+1], length, state)."""
+        dec_h, dec_c, memory, memory_proj = state
+        emb = F.relu(self.fs_decoder_embedding(dec_in))                                       # [1 x Ds]
+        if dropout:
+            emb = self.fs_decoder_embedding_drop(emb)
+        attn = self._calculate_attention(dec_h, memory_proj)                                  # [Tz]
+        context = (attn.unsqueeze(1) * memory).sum(dim=0, keepdim=True)                       # [1 x 2Ds]
+        mixed = F.relu(self.fs_decoder_attn_combine(torch.cat((emb, context), 1)).unsqueeze(0))  # [1 x 1 x Ds]
+        dec_out, (dec_h, dec_c) = self.fs_decoder_lstm(mixed, (dec_h, dec_c))
+        word_logits = self.fs_decoder_transcript(dec_out)                                     # [1 x 1 x M+1]
+        length = self.fs_decoder_length(F.relu(torch.cat((mixed, word_logits), 2))).squeeze()
+        return F.log_softmax(word_logits.squeeze(0), dim=1), length, (dec_h, dec_c, memory, memory_proj)
 
     def _decoder_param_list(self):
         """The 23 tensors of _lib.DECODER_PARAM_FIELDS, in that order (cached like WaveNetBlock.ordered_parameters: every entry's

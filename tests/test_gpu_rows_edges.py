@@ -178,3 +178,51 @@ def test_the_operators_called_by_name():
     listed = dict(teacher_values=values, teacher_index=index, teacher_lse=lse)
     assert torch.equal(ops.distill_loss(student=s, **listed), ops.distill_loss(s, values, index, lse))
     assert all(torch.equal(a, b) for a, b in zip(ops.distill_loss_and_grad(student=s, **listed), ops.distill_loss_and_grad(s, values, index, lse)))
+
+
+# ------------------------------------------------------------------------------------------------ in the model
+def a_model(hidden):
+    from mucon_amd.config import get_cfg_defaults, update_config
+    from mucon_amd.mucon.models import create_model
+    from test_gpu_model import seeded_value
+
+    over = ["model.fs.encoder.hidden_size", str(hidden), "model.fs.decoder.hidden_size", str(hidden)]
+    model = create_model(update_config(get_cfg_defaults(), [], [over]), num_classes=48, max_decoding_steps=31, input_feature_size=2048)
+    with torch.no_grad():
+        for name, p in model.named_parameters():
+            p.copy_(torch.from_numpy(seeded_value(name, p.shape).astype(np.float32)))
+    return model.cuda().eval()
+
+
+@pytest.mark.parametrize("hidden", [128, 64])
+def test_a_transcript_drawn_by_the_module_decoder(hidden, monkeypatch):
+    """native_decoder = False, and a decoder narrower than the native one's: the module's steps, with temperature 0 its greedy words, with uniforms the row oracle's
+    draws from its rows over the words before."""
+    from mucon_amd import ops
+    from test_gpu_model import make_batch
+
+    model, batch = a_model(hidden), make_batch(640, 5).to("cuda")
+    model.native_decoder = hidden != 128
+    u = torch.rand(31, generator=torch.Generator().manual_seed(3))
+
+    def no_native(*args, **kw):
+        raise AssertionError("the native decoder was called")
+
+    monkeypatch.setattr(ops, "decoder_forward", no_native)
+    model.set_teacher_forcing(False)
+    with torch.no_grad():
+        greedy = model.forward(batch).transcript.argmax(dim=1).tolist()
+    words, logp = model.sample_transcript(batch, u.cuda(), temperature=0.0)
+    assert words == greedy and not logp.any()
+    words, logp = model.sample_transcript(batch, u.cuda(), temperature=1.5, top_p=0.95)
+    assert len(words) == len(logp) and (words[-1] == model.EOS_token_id or len(words) == 31)
+    model.set_teacher_forcing(True)
+    with torch.no_grad():
+        given = torch.tensor([49] + words[:-1]).cuda()
+        rows, _ = model.sequence_generation_forward(model.temporal_modeling_forward(input=batch.feats), len(words), given, given)
+    check_drawn(words, logp.cpu(), host(torch.cat(rows)), u, (1.5, 0, np.float32(0.95).item(), 0.0))
+    if hidden == 128:
+        monkeypatch.undo()
+        model.native_decoder = True
+        again, _ = model.sample_transcript(batch, u.cuda(), temperature=1.5, top_p=0.95)
+        assert again == words      # (the rows agree to fp32, the uniforms are not at a border)
