@@ -415,9 +415,9 @@ class MuCon(nn.Module):
             logps.append(word_logp)
             words[s + 1] = word.clamp(min=0)      # (-1, a row without a distribution, is no embedding)
         out = torch.stack(drawn).tolist()
-        if -1 in out:
-            raise RuntimeError("sample_transcript: the decoder's outputs are not finite")
         n = out.index(self.EOS_token_id) + 1 if self.EOS_token_id in out else steps
+        if -1 in out[:n]:
+            raise RuntimeError("sample_transcript: the decoder's outputs are not finite")
         return out[:n], torch.stack(logps[:n])
 
     # ------------------------------------------------------------------------------ s-head

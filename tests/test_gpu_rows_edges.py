@@ -226,3 +226,20 @@ def test_a_transcript_drawn_by_the_module_decoder(hidden, monkeypatch):
         model.native_decoder = True
         again, _ = model.sample_transcript(batch, u.cuda(), temperature=1.5, top_p=0.95)
         assert again == words      # (the rows agree to fp32, the uniforms are not at a border)
+
+
+def test_what_is_drawn_behind_the_end_mark_does_not_count(monkeypatch):
+    """A row without a distribution (token -1) is an error in front of the end mark, nothing behind it."""
+    from mucon_amd import ops
+    from test_gpu_model import make_batch
+
+    model, batch = a_model(128), make_batch(640, 5).to("cuda")
+    for drawn, words in (([3, 7, 48, -1, 5], [3, 7, 48]), ([3, -1, 48, 1, 5], None), ([3, 7, 1, 1, -1], None)):
+        left = iter(drawn)
+        monkeypatch.setattr(ops, "sample_logits", lambda *a: (torch.tensor(next(left), device="cuda"), torch.tensor(-0.5, device="cuda")))
+        if words is None:
+            with pytest.raises(RuntimeError, match="not finite"):
+                model.sample_transcript(batch, torch.rand(5).cuda())
+        else:
+            got, logp = model.sample_transcript(batch, torch.rand(5).cuda())
+            assert got == words and len(logp) == len(words)
