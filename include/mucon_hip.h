@@ -513,7 +513,7 @@ int mucon_adam_clip_step(int32_t n_tensors, const mucon_adam_tensor *tensors, in
 #define MUCON_ROWS_MAX_SHORT 67108863
 
 /* The first k (1 .. 1,024) elements of each row's order -- values [rows][k] in the logits' type, index [rows][k] -- and lse [rows] =
- * log sum_j exp(x_j / temperature) over the whole row: the form in which a teacher's answers are kept for mucon_distill_*. */
+ * log sum_j exp(x_j / temperature) over the whole row: the form in which a teacher's answers are kept for mucon_distill_*.  temperature: 1e-30 .. 1e30. */
 size_t mucon_top_logits_workspace_bytes(int32_t type, int64_t rows, int32_t vocab, int32_t k);      /* may be 0 */
 int mucon_top_logits(int32_t type, int64_t rows, int32_t vocab, int64_t row_stride, int32_t k, double temperature, const void *logits, void *values,
                      int32_t *index, float *lse, void *workspace, size_t workspace_bytes, void *stream);
@@ -530,7 +530,7 @@ typedef struct mucon_distill_cfg {
     int32_t type, teacher_type; /* elements of the student (and its gradient) / of teacher_values */
     int32_t reduction;
     int32_t reserved;
-    double temperature;
+    double temperature;         /* 1e-30 .. 1e30 */
 } mucon_distill_cfg;
 size_t mucon_distill_workspace_bytes(const mucon_distill_cfg *cfg);
 /* teacher_values, teacher_index [rows][k]; teacher_lse [rows] or NULL.  Keeps each row's statistics in `workspace` for mucon_distill_bwd. */

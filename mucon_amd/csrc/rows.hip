@@ -38,6 +38,10 @@ static int rows_check(const char *what, int type, int64_t rows, int vocab, int64
     return MUCON_OK;
 }
 
+// Of top logits and distillation.  Within these log2(e) / T and its products with the differences of a row's logits keep their bits in fp32 (beyond, 0 times infinity made
+// rows NaN).
+static bool temperature_ok(double t) { return t >= 1e-30 && t <= 1e30; }
+
 #define BY_TYPE(type, F, ...)       \
     switch (type) {                 \
         case F32: F(F32, __VA_ARGS__); break; \
@@ -78,7 +82,7 @@ extern "C" int mucon_top_logits(int32_t type, int64_t rows, int32_t vocab, int64
     int rc = rows_check("top_logits", type, rows, vocab, row_stride);
     if (rc != MUCON_OK) return rc;
     if (k < 1 || k > MAX_K || k > vocab) return rfail(MUCON_E_ARG, "top_logits: k = %d of %d elements (1 .. min(vocab, %d))", k, vocab, MAX_K);
-    if (!(temperature > 0.0) || !isfinite(temperature)) return rfail(MUCON_E_ARG, "top_logits: temperature %g", temperature);
+    if (!temperature_ok(temperature)) return rfail(MUCON_E_ARG, "top_logits: temperature %g (1e-30 .. 1e30)", temperature);
     if (rows == 0) return MUCON_OK;
     if (!logits || !values || !index || !lse) return rfail(MUCON_E_ARG, "top_logits: null pointer argument");
     TopArgs a{logits, row_stride, vocab, k, temperature, values, index, lse};
@@ -124,7 +128,7 @@ static int distill_check(const mucon_distill_cfg *cfg) {
     if (rc != MUCON_OK) return rc;
     if (cfg->teacher_type < 0 || cfg->teacher_type > 2) return rfail(MUCON_E_ARG, "distill: teacher element type %d", cfg->teacher_type);
     if (cfg->k < 1 || cfg->k > MAX_K) return rfail(MUCON_E_ARG, "distill: %d listed entries a row (1 .. %d)", cfg->k, MAX_K);
-    if (!(cfg->temperature > 0.0) || !isfinite(cfg->temperature)) return rfail(MUCON_E_ARG, "distill: temperature %g", cfg->temperature);
+    if (!temperature_ok(cfg->temperature)) return rfail(MUCON_E_ARG, "distill: temperature %g (1e-30 .. 1e30)", cfg->temperature);
     if (cfg->reduction < 0 || cfg->reduction > 2) return rfail(MUCON_E_ARG, "distill: reduction %d (0 none, 1 sum, 2 mean)", cfg->reduction);
     if (cfg->rows < 1) return rfail(MUCON_E_ARG, "distill: no rows");
     return MUCON_OK;

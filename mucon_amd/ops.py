@@ -909,7 +909,7 @@ def _top_workspace_bytes(ty, rows, vocab, k):      # (a function of the sizes al
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     """The k largest logits of every row of `logits` [..., V] (float32, bfloat16 or float16; V up to 262,144, k up to 1,024) in order -- larger first, equal
     values by the lower index, -0 equal to +0, NaN above +inf -- and log sum exp(logits / temperature) of the whole rows: what distill_loss takes of a
-    teacher.  The values are the logits themselves (not divided by the temperature).  No gradient."""
+    teacher.  The values are the logits themselves (not divided by the temperature, 1e-30 .. 1e30).  No gradient."""
     lib = _lib.load()
     x, ty, rows, vocab, stride = _as_rows(logits, "top_logits")
     k = int(k)
@@ -1008,7 +1008,7 @@ class _DistillFn(torch.autograd.Function):
 def distill_loss(student: torch.Tensor, teacher_values: torch.Tensor, teacher_index: torch.Tensor, teacher_lse: Optional[torch.Tensor] = None,
                  temperature: float = 1.0, weight: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
     """Distillation of `student` [..., V] (logits; float32, bfloat16 or float16) from a teacher's top logits (top_logits): temperature^2 times the
-    Kullback-Leibler divergence of the student's distribution from the teacher's, both at `temperature`.
+    Kullback-Leibler divergence of the student's distribution from the teacher's, both at `temperature` (1e-30 .. 1e30).
 
     teacher_values, teacher_index [..., K] (int32; an index outside [0, V) is an empty entry).  Without teacher_lse the teacher is the softmax over its listed
     logits; with it (float32 [...], taken at the same temperature) the listed tokens have their own probabilities and all other tokens share the rest as one event.

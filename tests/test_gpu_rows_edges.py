@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import rows as orow
-from test_gpu_rows import U, check_distill, check_drawn, cuda, host, rows_of
+from test_gpu_rows import U, check_distill, check_drawn, cuda, host, rows_of, sum_error
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -243,3 +243,25 @@ def test_what_is_drawn_behind_the_end_mark_does_not_count(monkeypatch):
         else:
             got, logp = model.sample_transcript(batch, torch.rand(5).cuda())
             assert got == words and len(logp) == len(words)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [48, 200, 900, 9000, 40000])
+@pytest.mark.parametrize("T", [1e-30, 1e-6, 1e4, 1e30])      # (a gradient of T p: 65,504 is the largest of fp16)
+def test_the_ends_of_the_temperatures(V, dtype, T):
+    """Masked rows at the smallest and largest temperatures: one token or all of them alike."""
+    from mucon_amd import ops
+
+    x = rows_of("masked", 3, V, dtype, 4)
+    top = ops.top_logits(x.cuda(), 2, T)
+    values, index, lse = orow.top(host(x), 2, T)
+    assert np.array_equal(top.index.cpu().numpy(), index)
+    assert np.allclose(top.lse.cpu().numpy(), lse, rtol=U, atol=sum_error(V))
+    if T > 1e18:      # (T^2 L leaves fp32)
+        return
+    for given in (None, torch.from_numpy(np.float32(lse)) if T > 1 else None):      # (at the small ones a step of the log-sum-exp in fp32 is 1 and more: no distribution)
+        leaf = x.cuda().requires_grad_(True)
+        values = torch.from_numpy(host(top.values))
+        loss = ops.distill_loss(leaf, *cuda(values, top.index, given), temperature=T, reduction="none")
+        grad, = torch.autograd.grad(loss.sum(), leaf)
+        check_distill(loss.detach(), grad, x, values, top.index.cpu(), given, None, T, "none")

@@ -159,3 +159,17 @@ def test_every_argument_may_be_given_by_name():
             fn(**kw)
         with pytest.raises(TypeError, match="logits|student"):
             fn(**{name: v for name, v in kw.items() if v is not x})
+
+
+@pytest.mark.parametrize("temperature", [1e-300, 1e-46, 9e-31, 1.1e30, 1e46, 1e300])
+def test_temperatures_whose_inverse_leaves_fp32_are_refused(temperature):
+    """log2(e) / T is infinite or 0 in fp32 at the outer ones: 0 times infinity, a row of NaN."""
+    from mucon_amd import _lib
+
+    lib = _lib.load()
+    assert lib.mucon_top_logits(0, 2, 8, 8, 2, temperature, 64, 64, 64, 64, 0, 0, None) == _lib.E_ARG
+    assert b"temperature" in lib.mucon_last_error()
+    cfg = _cfg(temperature=temperature)
+    assert lib.mucon_distill_workspace_bytes(ctypes.byref(cfg)) == 0 and b"temperature" in lib.mucon_last_error()
+    for inside in (1e-30, 1e30):
+        assert lib.mucon_distill_workspace_bytes(ctypes.byref(_cfg(temperature=inside))) > 0
