@@ -13,7 +13,6 @@ namespace rows {
 enum { F32 = 0, BF16 = 1, F16 = 2 };
 constexpr int MAX_VOCAB = 1 << 18;   // a listed token's bit lies in LDS (32 KB), sums of 2^44-fold weights stay below 2^62
 constexpr int MAX_K = 1024;
-constexpr float LOG2E = 1.4426950408889634f;
 
 typedef unsigned long long u64;
 typedef uint32_t u32v4_1 __attribute__((ext_vector_type(4), aligned(2)));   // a 16-byte vector at a 2-byte border
@@ -180,8 +179,61 @@ struct RowIn {
     }
 };
 
-// the largest element of a vector, NaN if there is one
+// NaN if either is
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// ---- exp(d / T) of d = x - m <= 0 (or -inf, or NaN): 2^(d c), c = log2(e) / T ----
+// c in one fp32 number is off by the same share for every element of a row -- 1.3e-8 at T = 1, 3e-8 at most --, which moves the row's sum by that share of its mean exponent
+// (5e-8 over 50,000 tokens, three times what the sum's rounding leaves).  So c = hi + lo, hi rounded towards 0: lo > 0 keeps -inf times both -inf.  d c is rounded once: a weight
+// is off by |d c| / 2 steps of 2^-24, of either sign from element to element (a second fp32 number for the rounding, eight instructions instead of four, brought the losses' and
+// gradients' errors no lower -- 2.1e-8 and 2.5e-8 of themselves, 2,048 x 50,001 fp32 -- and 2,048 x 50,001 from 77 to 80 us).
+struct Exponent {
+    float hi, lo;
+};
+inline Exponent exponent_of(double temperature) {
+    const double c = 1.4426950408889634 / temperature;
+    float hi = (float)c;
+    if ((double)hi > c) hi = nextafterf(hi, 0.f);
+    return Exponent{hi, fmaxf((float)(c - (double)hi), 1.17549435e-38f)};
+}
+__device__ __forceinline__ float weight_of(float d, const Exponent &c) { return __builtin_amdgcn_exp2f(fmaf(d, c.hi, d * c.lo)); }
+// The weights of a vector's elements against m, added up: two or three fp32 roundings of half a step, of either sign; the vectors are summed in 64 bits
+template <int TY>
+__device__ __forceinline__ double weights_of(const Vec &v, float m, const Exponent &c) {
+    constexpr int N = El<TY>::N;
+    float w[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = weight_of(value_of<TY>(v, e) - m, c);
+#pragma unroll
+    for (int n = N / 2; n >= 1; n >>= 1)
+#pragma unroll
+        for (int e = 0; e < n; ++e) w[e] += w[e + n];
+    return (double)w[0];
+}
+
+// 2^t in 64 bits, |t| up to 1100: the nearest power of two times the exponential's series to the 11th power, off by 6e-15 of itself at most
+__device__ __forceinline__ double exp2_of(double t) {
+    const double n = rint(t), f = (t - n) * 0.69314718055994530942;
+    double p = 2.505210838544172e-8;
+    p = fma(p, f, 2.755731922398589e-7);
+    p = fma(p, f, 2.7557319223985893e-6);
+    p = fma(p, f, 2.48015873015873e-5);
+    p = fma(p, f, 1.984126984126984e-4);
+    p = fma(p, f, 1.3888888888888889e-3);
+    p = fma(p, f, 8.333333333333333e-3);
+    p = fma(p, f, 4.1666666666666664e-2);
+    p = fma(p, f, 0.16666666666666666);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.0);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n);
+}
+__device__ __forceinline__ double exp_of(double d) {      // e^d
+    const double t = d * 1.4426950408889634;
+    return exp2_of(t < -1100.0 ? -1100.0 : t > 1100.0 ? 1100.0 : t);      // (NaN stays)
+}
+
+// the largest element of a vector, NaN if there is one
 template <int TY>
 __device__ __forceinline__ float largest(const Vec &v) {
     float m = value_of<TY>(v, 0);

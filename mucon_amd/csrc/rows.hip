@@ -85,7 +85,7 @@ extern "C" int mucon_top_logits(int32_t type, int64_t rows, int32_t vocab, int64
     if (!temperature_ok(temperature)) return rfail(MUCON_E_ARG, "top_logits: temperature %g (1e-30 .. 1e30)", temperature);
     if (rows == 0) return MUCON_OK;
     if (!logits || !values || !index || !lse) return rfail(MUCON_E_ARG, "top_logits: null pointer argument");
-    TopArgs a{logits, row_stride, vocab, k, temperature, values, index, lse};
+    TopArgs a{logits, row_stride, vocab, k, temperature, exponent_of(temperature), values, index, lse};
     hipStream_t s = static_cast<hipStream_t>(stream);
     Slices sl = plan_slices(type, rows, vocab, k);
     if (sl.count > 1) {
@@ -155,6 +155,8 @@ static DistillArgs distill_args(const mucon_distill_cfg *cfg, const void *studen
     a.k = cfg->k;
     a.tt = cfg->teacher_type;
     a.temperature = cfg->temperature;
+    a.it = 1.0 / cfg->temperature;
+    a.c = exponent_of(cfg->temperature);
     char *w = static_cast<char *>(ws);
     a.losses = reinterpret_cast<float *>(w + distill_loss_off(cfg->rows));
     a.stat = reinterpret_cast<DistillRow *>(w + distill_stat_off());

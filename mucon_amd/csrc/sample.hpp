@@ -189,23 +189,6 @@ struct Weigh {
     double top, octaves;      // the largest logit; log2(e) / T
     __device__ __forceinline__ Weigh(float top_, double it) : top((double)top_), octaves(it * 1.4426950408889634) {}
     __device__ __forceinline__ double below(float x) const { return fmax(((double)x - top) * octaves, -100.0); }     // log2 of the weight, down to where nothing is left
-    // 2^t, t in [-100, 0]: the nearest power of two times the exponential's series to the 11th power, off by 6e-15 of itself at most
-    __device__ static __forceinline__ double exp2_of(double t) {
-        const double n = rint(t), f = (t - n) * 0.69314718055994530942;
-        double p = 2.505210838544172e-8;
-        p = fma(p, f, 2.755731922398589e-7);
-        p = fma(p, f, 2.7557319223985893e-6);
-        p = fma(p, f, 2.48015873015873e-5);
-        p = fma(p, f, 1.984126984126984e-4);
-        p = fma(p, f, 1.3888888888888889e-3);
-        p = fma(p, f, 8.333333333333333e-3);
-        p = fma(p, f, 4.1666666666666664e-2);
-        p = fma(p, f, 0.16666666666666666);
-        p = fma(p, f, 0.5);
-        p = fma(p, f, 1.0);
-        p = fma(p, f, 1.0);
-        return ldexp(p, (int)n);
-    }
     __device__ __forceinline__ double weight(float x) const { return exp2_of(below(x)); }
     __device__ static __forceinline__ u64 to_units(double w) { return (u64)(w * UNIT + 0.5); }
     __device__ __forceinline__ u64 units(float x) const { return to_units(weight(x)); }
@@ -603,7 +586,7 @@ __device__ void draw_by_bins(RowIn<TY, NT, 0> &in, const Drawing &d, float top, 
     in.each([&](const Vec &v, int i) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const double t = wg.below(value_of<TY>(v, e)), w = Weigh::exp2_of(t);
+            const double t = wg.below(value_of<TY>(v, e)), w = exp2_of(t);
             const u64 q = Weigh::to_units(w);
             const int b = min((int)(t * -BINS_PER_OCTAVE), BINS - 1);
             if (i * N + e < in.vocab) {

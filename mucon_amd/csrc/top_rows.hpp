@@ -289,6 +289,7 @@ struct TopArgs {
     long long stride;
     int vocab, k;
     double temperature;
+    Exponent c;
     void *values;
     int32_t *index;
     float *lse;
@@ -296,7 +297,7 @@ struct TopArgs {
 
 template <int TY, int NT, int NV>
 __global__ __launch_bounds__(NT, NT == 512 ? 8 : 1) void top_rows_kernel(TopArgs a) {
-    constexpr int N = El<TY>::N, L = NT > 512 ? LIST : SHORT_LIST;
+    constexpr int L = NT > 512 ? LIST : SHORT_LIST;
     __shared__ SelectShared<L> sh;
     const long long r = blockIdx.x;
     RowIn<TY, NT, NV> in(row_at<TY>(a.x, r, a.stride), a.vocab);
@@ -305,13 +306,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 8 : 1) void top_rows_kernel(TopArgs
     const float m = block_reduce<NT, MaxNan>(mine, sh.f);
     double s = 0.0;
     if (isfinite(m)) {
-        const float c = (float)(1.4426950408889634 / a.temperature);
-        in.each([&](const Vec &v, int) {
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < N; ++e) sum += __builtin_amdgcn_exp2f((value_of<TY>(v, e) - m) * c);
-            s += (double)sum;
-        });
+        in.each([&](const Vec &v, int) { s += weights_of<TY>(v, m, a.c); });
         s = block_reduce<NT, Sum>(s, sh.d);
     }
     if (threadIdx.x == 0) a.lse[r] = isfinite(m) ? (float)((double)m / a.temperature + log(s)) : m;
@@ -343,10 +338,9 @@ struct Slices {
     u64 *kept;      // [rows][count][keep]
 };
 
-// The first k of slice `s` of row r, its largest element m and its sum of exp2((x - m) c)
+// The first k of slice `s` of row r, its largest element m and its sum of exp((x - m) / T)
 template <int TY, int NT>
-__device__ void cut_slice(const char *row, int vocab, long long r, int s, int k, float c, const Slices &sl, SelectShared<LIST> &sh) {
-    constexpr int N = El<TY>::N;
+__device__ void cut_slice(const char *row, int vocab, long long r, int s, int k, const Exponent &c, const Slices &sl, SelectShared<LIST> &sh) {
     const int first = s * sl.length, length = min(sl.length, vocab - first);
     Slices::Part &part = sl.part[r * sl.count + s];
     RowIn<TY, NT, CUT, true> in(row + (long long)first * sizeof(typename El<TY>::type), length);
@@ -355,12 +349,7 @@ __device__ void cut_slice(const char *row, int vocab, long long r, int s, int k,
     const float m = block_reduce<NT, MaxNan>(mine, sh.f);
     double sum = 0.0;
     if (isfinite(m)) {
-        in.each([&](const Vec &v, int) {
-            float w = 0.f;
-#pragma unroll
-            for (int e = 0; e < N; ++e) w += __builtin_amdgcn_exp2f((value_of<TY>(v, e) - m) * c);
-            sum += (double)w;
-        });
+        in.each([&](const Vec &v, int) { sum += weights_of<TY>(v, m, c); });
         sum = block_reduce<NT, Sum>(sum, sh.d);
     }
     k = min(k, length);
@@ -392,7 +381,7 @@ template <int TY, int NT>
 __global__ __launch_bounds__(NT) void top_cut_kernel(TopArgs a, Slices sl) {
     __shared__ SelectShared<LIST> sh;
     const long long r = blockIdx.x / sl.count;
-    cut_slice<TY, NT>(row_at<TY>(a.x, r, a.stride), a.vocab, r, (int)(blockIdx.x % sl.count), a.k, (float)(1.4426950408889634 / a.temperature), sl, sh);
+    cut_slice<TY, NT>(row_at<TY>(a.x, r, a.stride), a.vocab, r, (int)(blockIdx.x % sl.count), a.k, a.c, sl, sh);
 }
 template <int TY, int NT>
 __global__ __launch_bounds__(NT) void top_join_kernel(TopArgs a, Slices sl) {
@@ -469,7 +458,7 @@ __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a, long long row
     u64 c[E];
     sorted_row<TY, E>(row, a.vocab, c);
     const uint32_t top = __shfl(key_of(c[0]), 0);
-    const float m = value_of_key<TY>(top), scale = (float)(1.4426950408889634 / a.temperature);
+    const float m = value_of_key<TY>(top);
     typedef typename El<TY>::type T;
     double s = 0.0;
 #pragma unroll
@@ -480,7 +469,7 @@ __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a, long long row
             a.index[r * a.k + place] = at;
             static_cast<T *>(a.values)[r * a.k + place] = reinterpret_cast<const T *>(row)[at];
         }
-        if (place < a.vocab) s += (double)__builtin_amdgcn_exp2f((value_of_key<TY>(key_of(c[e])) - m) * scale);
+        if (place < a.vocab) s += (double)weight_of(value_of_key<TY>(key_of(c[e])) - m, a.c);
     }
     s = wave_reduce<Sum>(s);
     if (lane == 0) a.lse[r] = top == key_top<TY>() ? NAN : isinf(m) ? m : (float)((double)m / a.temperature + log(s));

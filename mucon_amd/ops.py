@@ -975,7 +975,7 @@ _EAGER_STREAM = "mucon_amd: stream of the eager graph"
 
 
 class _DistillFn(torch.autograd.Function):
-    """Forward: the rows' losses and, per row, what the gradient needs (32 bytes); backward: one pass over the student's rows."""
+    """Forward: the rows' losses and, per row, what the gradient needs (40 bytes); backward: one pass over the student's rows."""
 
     @staticmethod
     def forward(ctx, student, values, index, lse, weight, temperature, reduction):

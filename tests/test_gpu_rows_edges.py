@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import rows as orow
-from test_gpu_rows import U, check_distill, check_drawn, cuda, host, rows_of, sum_error
+from test_gpu_rows import U, check_distill, check_drawn, cuda, distill_case, host, rows_of, sum_error
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -147,6 +147,25 @@ def test_distill_far_rows_whose_unlisted_tokens_rise(V, dtype):
     check_distill(loss, grad, s, values, index, lse, None, T, "none")
 
 
+@pytest.mark.parametrize("V", [7, 48, 900, 40000])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_where_every_unlisted_token_is_masked(V, dtype):
+    """A vocabulary masked down to the listed tokens, whose logits lie far below, around and above 0: there is no rest term, and no gradient elsewhere."""
+    from mucon_amd import ops
+
+    for T in (0.004, 1.0):
+        s, values, index, lse = far_case(V, dtype, T, 3, [0.0, 0.25, 0.5])
+        for shift in (-60.0, 0.0, 60.0):
+            x = torch.full_like(s, -math.inf).scatter(1, index.long(), (s.float().gather(1, index.long()) + shift).to(dtype))
+            leaf = x.cuda().requires_grad_(True)
+            loss = ops.distill_loss(leaf, *cuda(values, index, lse), temperature=T, reduction="none")
+            grad, = torch.autograd.grad(loss.sum(), leaf)
+            check_distill(loss.detach(), grad, x, values, index, lse, None, T, "none")
+            loss, grad = ops.distill_loss_and_grad(x.cuda(), *cuda(values, index, lse), temperature=T, reduction="none")
+            check_distill(loss, grad, x, values, index, lse, None, T, "none")
+            assert not grad[x.isneginf().cuda()].any()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_distill_with_a_rest_at_a_low_temperature_and_far_from_zero(dtype):
     """Logits around 60 at temperature 1/20 with the teacher's log-sum-exp given: near 1,200, where its own step in fp32 is 2^-13, which enters 1 - sum p as it is given."""
@@ -165,6 +184,50 @@ def test_distill_with_a_rest_at_a_low_temperature_and_far_from_zero(dtype):
         check_distill(loss.detach(), grad, s, values, index, lse, None, 0.05, "sum")
         loss, grad = ops.distill_loss_and_grad(s.cuda(), *cuda(values, index, lse), temperature=0.05, reduction="sum")
         check_distill(loss, grad, s, values, index, lse, None, 0.05, "sum")
+
+
+def plain_distill(s, values, index, lse, T):
+    """The rows' losses in torch operations: exponentials in fp32, sums and the few listed entries in 64 bits."""
+    at, top = index.long(), s.detach().max(dim=1, keepdim=True).values
+    e = ((s - top) / T).exp()
+    log_total = e.sum(dim=1, dtype=torch.float64).log()
+    log_q = (s.gather(1, at).double() - top.double()) / T - log_total[:, None]
+    log_p = values.double() / T - lse.double()[:, None]
+    p = log_p.exp()
+    rest = 1.0 - p.sum(dim=1)
+    outside = torch.where(torch.zeros_like(e).scatter_(1, at, 1.0) > 0, torch.zeros_like(e), e).sum(dim=1, dtype=torch.float64)
+    return ((p * (log_p - log_q)).sum(dim=1) + rest * (rest.log() - outside.log() + log_total)) * T * T
+
+
+@pytest.mark.parametrize("rows,V", [(512, 49), (256, 300), (128, 3000), (64, 20001), (48, 50001)])
+@pytest.mark.parametrize("T", [1.0, 2.0, 1.3, 0.7])
+def test_distill_in_fp32_is_as_near_the_definition_as_the_plain_form(rows, V, T):
+    """The root mean square of the rows' losses' errors and of the gradient's elements', each against 64 bits, are at most those of the same formula in torch's fp32 operations: a
+    constant of the exponent in one fp32 number (T = 1, 2), or coefficients in fp32, show here as a bias.  (A tenth more for chance: both hold the final rounding, whose mean square over
+    48 losses varies by 1 / sqrt(5 / 4 x 48) = 0.13, a root of 0.065.)"""
+    from mucon_amd import ops
+
+    s, values, index, lse, _ = distill_case(rows, V, 16, torch.float32, torch.float32, True, False, V, T)
+    s, values, index, lse = cuda(s, values, index, lse)
+    exact = s.double().requires_grad_(True)
+    log_q = torch.log_softmax(exact / T, 1)
+    log_p = values.double() / T - lse.double()[:, None]
+    p = log_p.exp()
+    rest = 1.0 - p.sum(1)
+    unlisted = torch.ones_like(log_q).scatter(1, index.long(), 0.0)
+    want = ((p * (log_p - log_q.gather(1, index.long()))).sum(1) + rest * (rest.log() - (unlisted * log_q.exp()).sum(1).log())) * T * T
+    want_grad, = torch.autograd.grad(want.mean(), exact)
+
+    def errors(loss, grad):
+        return [float((a.double() - b).norm() / b.norm()) for a, b in ((loss, want.detach()), (grad, want_grad))]
+
+    plain = s.clone().requires_grad_(True)
+    of_plain = errors(plain_distill(plain, values, index, lse, T).detach().float(), torch.autograd.grad(plain_distill(plain, values, index, lse, T).mean().float(), plain)[0])
+    leaf = s.clone().requires_grad_(True)
+    loss = ops.distill_loss(leaf, values, index, lse, temperature=T, reduction="none").detach()
+    for grad in (torch.autograd.grad(ops.distill_loss(leaf, values, index, lse, temperature=T), leaf)[0], ops.distill_loss_and_grad(s, values, index, lse, temperature=T)[1]):
+        for mine, theirs in zip(errors(loss, grad), of_plain):
+            assert mine <= 1.1 * theirs, (errors(loss, grad), of_plain)
 
 
 # ------------------------------------------------------------------------------------------------ calls
@@ -262,6 +325,7 @@ def test_the_ends_of_the_temperatures(V, dtype, T):
     for given in (None, torch.from_numpy(np.float32(lse)) if T > 1 else None):      # (at the small ones a step of the log-sum-exp in fp32 is 1 and more: no distribution)
         leaf = x.cuda().requires_grad_(True)
         values = torch.from_numpy(host(top.values))
+        values[0] = values[0, 0]      # (the largest twice: half a probability each)
         loss = ops.distill_loss(leaf, *cuda(values, top.index, given), temperature=T, reduction="none")
         grad, = torch.autograd.grad(loss.sum(), leaf)
         check_distill(loss.detach(), grad, x, values, top.index.cpu(), given, None, T, "none")
