@@ -73,6 +73,50 @@ def test_draws_of_logits_at_the_end_of_fp32():
             check_drawn(token.cpu(), logp.cpu(), host(x), u, (np.float32(T).item(), k, np.float32(p).item(), 0.0))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [48, 200, 900, 3000, 9000, 70000])
+def test_few_tokens_allowed_and_more_asked_for(V, dtype):
+    """Rows of which 20 tokens are above -inf, with top_k and k beyond that: all of them, then (of top_logits) the masked ones by their index."""
+    from mucon_amd import ops
+
+    g = torch.Generator().manual_seed(V)
+    x = torch.full((4, V), -math.inf)
+    for r in range(4):
+        x[r, torch.randperm(V, generator=g)[:20]] = torch.randn(20, generator=g)
+    x = x.to(dtype)
+    for k in (19, 20, 21, min(V, 50), min(V, 1000)):
+        top = ops.top_logits(x.cuda(), k, 0.8)
+        values, index, lse = orow.top(host(x), k, 0.8)
+        assert np.array_equal(top.index.cpu().numpy(), index) and np.array_equal(host(top.values), values)
+        assert np.allclose(top.lse.cpu().numpy(), lse, rtol=U, atol=sum_error(V))
+    u = torch.tensor([0.0, 0.3, 0.7, 1.0 - 2.0 ** -24])
+    for k in (19, 20, 21, 50, 1000, 5000):
+        for p, m in ((1.0, 0.0), (0.8, 0.0), (1.0, 0.2), (0.9, 0.05)):
+            token, logp = ops.sample_logits(*cuda(x, u), 0.8, k, p, m)
+            check_drawn(token.cpu(), logp.cpu(), host(x), u, (np.float32(0.8).item(), k, np.float32(p).item(), np.float32(m).item()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["flat", "ties", "normal"])
+@pytest.mark.parametrize("V", [48, 200, 900, 3000, 9000, 70000])
+def test_rows_of_their_own_parameters_in_every_type(V, kind, dtype):
+    from mucon_amd import ops
+
+    if V == 70000 and kind == "ties":
+        pytest.skip("as 9,000")
+    rows = 16
+    x = rows_of(kind, rows, V, dtype, 7)
+    x[3, V // 3:] = -math.inf
+    g = torch.Generator().manual_seed(V)
+    T = torch.rand(rows, generator=g) * 2 + 0.3
+    k = torch.randint(0, 2 * min(V, 1500), (rows,), generator=g).to(torch.int32)
+    p, m = torch.rand(rows, generator=g) * 1.3, torch.rand(rows, generator=g) * 0.3
+    T[0], k[1], p[2], m[4], p[5], k[6] = 0.0, 0, 0.0, 1.0, -0.5, 1
+    u = torch.rand(rows, generator=g)
+    token, logp = ops.sample_logits(*cuda(x, u), *cuda(T, k, p, m))
+    check_drawn(token.cpu(), logp.cpu(), host(x), u, (T, torch.where(k >= V, torch.zeros_like(k), k), p, m))
+
+
 # ------------------------------------------------------------------------------------------------ distillation
 def far_case(V, dtype, T, seed, levels, rest_mass=0.5, rows=4):
     """Unlisted student logits within half a unit of 0, listed ones at `levels` (exact in every type); the teacher leaves `rest_mass` to the unlisted tokens."""
@@ -228,6 +272,32 @@ def test_distill_in_fp32_is_as_near_the_definition_as_the_plain_form(rows, V, T)
     for grad in (torch.autograd.grad(ops.distill_loss(leaf, values, index, lse, temperature=T), leaf)[0], ops.distill_loss_and_grad(s, values, index, lse, temperature=T)[1]):
         for mine, theirs in zip(errors(loss, grad), of_plain):
             assert mine <= 1.1 * theirs, (errors(loss, grad), of_plain)
+
+
+@pytest.mark.parametrize("rows,V,K", [(40, 49, 4), (9, 300, 16), (5, 4000, 40), (3, 20001, 64), (2, 131072, 64), (1, 262144, 1024)])
+@pytest.mark.parametrize("T", [1.0, 0.6])
+def test_distill_gradients_in_fp32_element_by_element(rows, V, K, T):
+    """An unlisted token's weight is exp2 of an exponent of t: the difference and the product round once each (2 t u ln 2 of the weight), exp2 to a step (2 u), the last product and the
+    result once (2 u).  The row's sum has that of its mean exponent, at most log2 V, and three roundings of a vector's; it enters every element in its share.  A listed token's own
+    terms are 64-bit."""
+    from mucon_amd import ops
+
+    s, values, index, lse, _ = distill_case(rows, V, K, torch.float32, torch.float32, True, False, V + K, T)
+    want = orow.distill(s, values, index, lse, T, None, "none")[1]
+    q = torch.softmax(s.double() / T, 1)
+    listed = torch.zeros_like(q).scatter(1, index.long(), 1.0) > 0
+    mo = torch.where(listed, torch.full_like(s, -math.inf), s).max(1, keepdim=True).values.double()
+    p = torch.exp(values.double() / T - lse.double()[:, None])
+    rest = (1.0 - p.sum(1, keepdim=True)).clamp(min=0)
+    share = T * (q + torch.where(listed, 0.0, rest * q / (q * ~listed).sum(1, keepdim=True)))
+    t = (mo - s.double()) / T / math.log(2)
+    of_sum = (2 * math.log(2) * math.log2(V) + 2 + 3) * U
+    bound = share * (of_sum + torch.where(listed, 0.0, (2 * math.log(2) * t + 4) * U)) + U * want.abs() + 1e-14
+    leaf = s.cuda().requires_grad_(True)
+    d = cuda(values, index, lse)
+    for grad in (torch.autograd.grad(ops.distill_loss(leaf, *d, temperature=T, reduction="sum"), leaf)[0], ops.distill_loss_and_grad(s.cuda(), *d, temperature=T, reduction="sum")[1]):
+        err = (grad.double().cpu() - want).abs()
+        assert bool((err <= bound).all()), float((err / bound).max())
 
 
 # ------------------------------------------------------------------------------------------------ calls
