@@ -45,11 +45,11 @@ __device__ __forceinline__ float quad_sum(float v) {   // the same bits in all f
     return v;
 }
 // acc += w * g.lo / acc += w * g.hi for both halves of a pair: two single FMAs each (the packed form with a broadcast operand is not used: build.py, COMMON)
-__device__ __forceinline__ void pk_fma_lo(f32x2 &acc, f32x2 w, f32x2 g) {
+__device__ __forceinline__ void fma_lo(f32x2 &acc, f32x2 w, f32x2 g) {
     acc[0] = __builtin_fmaf(w[0], g[0], acc[0]);
     acc[1] = __builtin_fmaf(w[1], g[0], acc[1]);
 }
-__device__ __forceinline__ void pk_fma_hi(f32x2 &acc, f32x2 w, f32x2 g) {
+__device__ __forceinline__ void fma_hi(f32x2 &acc, f32x2 w, f32x2 g) {
     acc[0] = __builtin_fmaf(w[0], g[1], acc[0]);
     acc[1] = __builtin_fmaf(w[1], g[1], acc[1]);
 }
@@ -327,14 +327,14 @@ __global__ __launch_bounds__(512) void lstm_recur_bwd_kernel(LstmWeights w, cons
         for (int r4 = 0; r4 < 8; ++r4) {
             const f32x4 gv = *reinterpret_cast<const f32x4 *>(&dgs[cur][rho * LSTM_SEG + r4 * 4]);   // (all eight reads in front, as in the forward: slower, 106 us against 103)
             const f32x2 g01 = {gv[0], gv[1]}, g23 = {gv[2], gv[3]};
-            pk_fma_lo(a0, wt[r4 * 4 + 0][0], g01);
-            pk_fma_lo(a1, wt[r4 * 4 + 0][1], g01);
-            pk_fma_hi(a0, wt[r4 * 4 + 1][0], g01);
-            pk_fma_hi(a1, wt[r4 * 4 + 1][1], g01);
-            pk_fma_lo(a0, wt[r4 * 4 + 2][0], g23);
-            pk_fma_lo(a1, wt[r4 * 4 + 2][1], g23);
-            pk_fma_hi(a0, wt[r4 * 4 + 3][0], g23);
-            pk_fma_hi(a1, wt[r4 * 4 + 3][1], g23);
+            fma_lo(a0, wt[r4 * 4 + 0][0], g01);
+            fma_lo(a1, wt[r4 * 4 + 0][1], g01);
+            fma_hi(a0, wt[r4 * 4 + 1][0], g01);
+            fma_hi(a1, wt[r4 * 4 + 1][1], g01);
+            fma_lo(a0, wt[r4 * 4 + 2][0], g23);
+            fma_lo(a1, wt[r4 * 4 + 2][1], g23);
+            fma_hi(a0, wt[r4 * 4 + 3][0], g23);
+            fma_hi(a1, wt[r4 * 4 + 3][1], g23);
         }
         float col[4] = {a0[0], a0[1], a1[0], a1[1]};
 #pragma unroll

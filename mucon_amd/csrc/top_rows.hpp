@@ -234,23 +234,21 @@ __device__ int select_first(ROW &in, int k, float mine, SelectShared<L> &sh) {
     }
     if (tid == 0) sh.n = 0;
     __syncthreads();
-    if (vocab <= L || k <= NT) {
-        in.each([&](const Vec &v, int i) {
-            if (!(largest<TY>(v) >= bound)) return;
+    in.each([&](const Vec &v, int i) {
+        if (!(largest<TY>(v) >= bound)) return;
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                if (value_of<TY>(v, e) >= bound && i * N + e < vocab) {
-                    const int at = atomicAdd(&sh.n, 1);
-                    if (at < L) sh.list[at] = composite(key_of<TY>(v, e), i * N + e);
-                }
+        for (int e = 0; e < N; ++e) {
+            if (value_of<TY>(v, e) >= bound && i * N + e < vocab) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < L) sh.list[at] = composite(key_of<TY>(v, e), i * N + e);
             }
-        });
-        __syncthreads();
-        const int n = sh.n;
-        if (n <= L) {
-            sort_list<NT, L>(sh.list, n, sh.sort);
-            return n;
         }
+    });
+    __syncthreads();
+    const int n = sh.n;
+    if (n <= L) {
+        sort_list<NT, L>(sh.list, n, sh.sort);
+        return n;
     }
     // the k-th largest value, bit by bit of its key
     uint32_t t = 0;
