@@ -81,7 +81,7 @@ __device__ __forceinline__ DistillRow finish_row(const ListSums &l, const TokenS
         *loss = l.A - B + (pr > 0.0 ? pr * (log_last - log_qr) : pr);
         const double P = l.S + pr;
         st.in = P / Z;
-        st.out = P * wo / Z - (pr > 0.0 ? pr / z.Zo : pr);
+        st.out = st.in * wo - (pr > 0.0 ? pr / z.Zo : pr);
         st.lp0 = lse;
     } else {
         *loss = l.S == 0.0 ? 0.0 : (l.A - B) / l.S - log_last;
@@ -342,8 +342,13 @@ template <int TY>
 __device__ __forceinline__ void grad_vector(const Vec &v, float base, const Exponent &c, const Factor &f, float *x) {
 #pragma unroll
     for (int e = 0; e < El<TY>::N; ++e) {
-        const float w = weight_of(value_of<TY>(v, e) - base, c);
-        x[e] = TY == F32 ? fmaf(w, f.hi, w * f.lo) : w * f.hi;
+        const float d = value_of<TY>(v, e) - base;
+        if (TY == F32) {
+            const float w = weight_of(d, c);
+            x[e] = fmaf(w, f.hi, w * f.lo);
+        } else {      // (rounded to 2^-9 or 2^-12 of itself: an exponent off by 2^-25 of its 60 or so does not reach it)
+            x[e] = f.hi * __builtin_amdgcn_exp2f(d * c.one);
+        }
     }
 }
 
@@ -465,17 +470,19 @@ __global__ __launch_bounds__(NT) void distill_stream_kernel(DistillArgs a) {
     double s = 0.0;
     for (int first = tid; first < nvec; first += NT * AHEAD) {
         Vec v[AHEAD];
-        uint32_t in[AHEAD];
         float top = -INFINITY;
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
             const int i = first + q * NT;
-            if (rest) in[q] = bits_at<TY>(list, i, nvec);
             if (i < nvec)
                 v[q] = load_vec<TY>(row, i, a.vocab);
             else
                 v[q] = Vec{{El<TY>::LOWEST, El<TY>::LOWEST, El<TY>::LOWEST, El<TY>::LOWEST}};
         }
+        uint32_t in[AHEAD];      // (read behind the loads, not between them)
+        if (rest)
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) in[q] = bits_at<TY>(list, first + q * NT, nvec);
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
             if (rest) hide_listed<TY>(v[q], in[q]);
@@ -563,18 +570,13 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillArgs a, int chun
     for (int i = tid; i < PER / 32; i += NT) bits[i] = 0;
     if (tid == 0) again = found = 0;
     __syncthreads();
-    // A thread's first entry is read while the row's loads are on their way.  The listed tokens' stores wait for the others' at the barrier.
-    int at = -1;
-    float t = 0.f, listed = 0.f;
+    // (a listed token's store waits for the others' at the barrier; which tokens are listed twice is looked for meanwhile.  Its entry's logits read here too, ahead of the barrier:
+    // 16,384 x 1,000 bf16 28 -> 32 us, the wave with the list holds up the others' stores)
     for (int k = tid; k < a.k; k += NT) {
         const int j = a.index[r * a.k + k];
         if (j < first || j - first >= PER || j >= a.vocab) continue;
         if (atomicOr(&bits[(j - first) >> 5], 1u << (j & 31)) >> (j & 31) & 1) again = 1;
         found = 1;
-        if (k != tid) continue;
-        at = j;
-        t = teacher_value(a.t, a.tt, r * a.k + k);
-        listed = value_of_bits<TY>(load_bits<TY>(row, j));
     }
     const Factor fout = factor_of(g * st.out);
 #pragma unroll
@@ -585,13 +587,9 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(DistillArgs a, int chun
     __syncthreads();
     if (!found) return;
     for (int k = tid; k < a.k; k += NT) {
-        if (k != tid) {
-            at = a.index[r * a.k + k];
-            if (at < first || at - first >= PER || at >= a.vocab) continue;
-            t = teacher_value(a.t, a.tt, r * a.k + k);
-            listed = value_of_bits<TY>(load_bits<TY>(row, at));
-        }
-        if (at < 0) continue;
+        const int at = a.index[r * a.k + k];
+        if (at < first || at - first >= PER || at >= a.vocab) continue;
+        const float t = teacher_value(a.t, a.tt, r * a.k + k), listed = value_of_bits<TY>(load_bits<TY>(row, at));
         double p = 0.0;
         if (again) {      // all entries of the token, in the list's order
             for (int q = 0; q < a.k; ++q)

@@ -189,12 +189,13 @@ __device__ __forceinline__ float maximum(float a, float b) { return __builtin_el
 // gradients' errors no lower -- 2.1e-8 and 2.5e-8 of themselves, 2,048 x 50,001 fp32 -- and 2,048 x 50,001 from 77 to 80 us).
 struct Exponent {
     float hi, lo;
+    float one;      // the nearest, where the weight itself is rounded to 16 bits
 };
 inline Exponent exponent_of(double temperature) {
     const double c = 1.4426950408889634 / temperature;
     float hi = (float)c;
     if ((double)hi > c) hi = nextafterf(hi, 0.f);
-    return Exponent{hi, fmaxf((float)(c - (double)hi), 1.17549435e-38f)};
+    return Exponent{hi, fmaxf((float)(c - (double)hi), 1.17549435e-38f), (float)c};
 }
 __device__ __forceinline__ float weight_of(float d, const Exponent &c) { return __builtin_amdgcn_exp2f(fmaf(d, c.hi, d * c.lo)); }
 // The weights of a vector's elements against m, added up: two or three fp32 roundings of half a step, of either sign; the vectors are summed in 64 bits
