@@ -447,7 +447,7 @@ __global__ __launch_bounds__(NT, NV <= 4 ? 8 : 1) void distill_row_kernel(Distil
 }
 
 // Longer rows: streamed, with a running maximum; GRAD: the row once more, from a cache, for its gradient.  Several such workgroups share a CU, so that one loads while
-// another adds up; a row held in the registers of one workgroup of 1,024 leaves the memory idle meanwhile (2,048 rows of 131,072 bf16: 345 us, so 263).
+// another adds up; a row held in the registers of one workgroup of 1,024 leaves the memory idle meanwhile (2,048 rows of 131,072 bf16: 345 us, so 254).
 template <int TY, int NT, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_stream_kernel(DistillArgs a) {
     constexpr int N = El<TY>::N, AHEAD = 4;

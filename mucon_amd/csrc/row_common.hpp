@@ -185,8 +185,8 @@ __device__ __forceinline__ float maximum(float a, float b) { return __builtin_el
 // ---- exp(d / T) of d = x - m <= 0 (or -inf, or NaN): 2^(d c), c = log2(e) / T ----
 // c in one fp32 number is off by the same share for every element of a row -- 1.3e-8 at T = 1, 3e-8 at most --, which moves the row's sum by that share of its mean exponent
 // (5e-8 over 50,000 tokens, three times what the sum's rounding leaves).  So c = hi + lo, hi rounded towards 0: lo > 0 keeps -inf times both -inf.  d c is rounded once: a weight
-// is off by |d c| / 2 steps of 2^-24, of either sign from element to element (a second fp32 number for the rounding, eight instructions instead of four, brought the losses' and
-// gradients' errors no lower -- 2.1e-8 and 2.5e-8 of themselves, 2,048 x 50,001 fp32 -- and 2,048 x 50,001 from 77 to 80 us).
+// is off by |d c| / 2 steps of 2^-24, of either sign from element to element (a second fp32 number for the rounding, eight instructions instead of four, left the losses' errors at
+// 2.1e-8 of themselves and brought the gradients' from 3.3e-8 to 3.0e-8, 50,001 fp32 tokens at T = 1; a forward of 2,048 x 50,001 went from 77 to 80 us).
 struct Exponent {
     float hi, lo;
     float one;      // the nearest, where the weight itself is rounded to 16 bits
@@ -247,7 +247,7 @@ struct MaxNan {
 };
 
 // vector i of a gradient row from fp32 values; past the caches, which hold the rows that are still to be read (2,048 rows of 131,072 bf16, loss and gradient: 315 -> 279 us,
-// and 263 with the second read of a row as its last)
+// 263 with the second read of a row as its last, 254 with its listed tokens' weights taken once)
 template <int TY>
 __device__ __forceinline__ void store_vec(char *row, int i, int vocab, const float *x) {
     constexpr int N = El<TY>::N;
